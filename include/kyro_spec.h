@@ -464,7 +464,9 @@ int kyro_chunk_attention(kyro_ctx* ctx, const kyro_chunk_params* p, const void* 
  * empty chunk leaves its whole row of scores_out as it was.
  *   q bf16 [T, Hq, D], lse fp32 [T, Hq]: those of kyro_chunk_attention
  *   scores, scores_out fp32 [B, Hkv, score_slots]; they may be the same
- * A sequence that needs more than score_slots sets KYRO_DEV_BAD_LENGTH.
+ * A sequence that needs more than score_slots sets KYRO_DEV_BAD_LENGTH.  Any
+ * table below 2^30 slots is taken (the attention, where lse comes from, takes
+ * 2^27).
  * Sums run in a fixed order: the same call gives the same bits. */
 size_t kyro_kv_scores_add_workspace_size(const kyro_chunk_params* p);
 int kyro_kv_scores_add(kyro_ctx* ctx, const kyro_chunk_params* p, const void* q,

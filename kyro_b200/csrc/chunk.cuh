@@ -6,6 +6,7 @@
 
 #include <atomic>
 
+#include "chunk_index.h"
 #include "kyro_internal.cuh"
 #include "ptx.cuh"
 #include "tcgen05.cuh"

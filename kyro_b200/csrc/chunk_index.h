@@ -1,0 +1,28 @@
+// chunk_index.h -- index arithmetic of the operators on packed prompt chunks
+// that has to hold at the limits of what they accept.  It compiles as CUDA
+// and as plain C++, so that a test can go through the limits on the CPU.
+#pragma once
+
+#include <stdint.h>
+
+#ifdef __CUDACC__
+#define KYRO_HD __host__ __device__ __forceinline__
+#else
+#define KYRO_HD inline
+#endif
+
+namespace kyro {
+namespace chunk {
+
+// The columns of a step of scores (tokens from tok0 on, `group` heads each)
+// that do not see a slot, which tokens from tok_min on see: the first so
+// many.  A slot of the context has tok_min = t - ctx, down to -2^30, so the
+// difference is cut at zero before it is multiplied; it is no more than the
+// slots of an item and the tokens of a step, 256 + 128 / group.
+KYRO_HD int hidden_cols(int tok_min, int tok0, int group) {
+  const int d = tok_min - tok0;
+  return d > 0 ? d * group : 0;
+}
+
+}  // namespace chunk
+}  // namespace kyro

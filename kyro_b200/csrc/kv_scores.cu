@@ -453,7 +453,7 @@ kv_scores_kernel(const __grid_constant__ CUtensorMap tmQ,
               sum_cols<32>(x, ls + c / 4, sl, acc);
             }
           } else {
-            const int cmin = (tok_min - tok0) * group;
+            const int cmin = kyro::chunk::hidden_cols(tok_min, tok0, group);
 #pragma unroll 1
             for (int c = 0; c < kTN / 2 && c0 + c < valid; c += 8) {
               uint32_t x[8];
