@@ -389,13 +389,15 @@ int kyro_rope_kv_write(kyro_ctx* ctx, const kyro_kv_params* p, int32_t num_new,
  * sequences are packed: chunk_starts (int32 [B + 1], on the device) says
  * that rows chunk_starts[b] .. chunk_starts[b+1]-1 are sequence b's new
  * tokens, at cache slots context_lens[b] + 0, 1, ...  A chunk may be empty.
- * Rows before chunk_starts[0] and from chunk_starts[B] on are padding: they
- * are not read, and what lies there in an output is left as it was.  A
- * sequence whose chunk_starts entries decrease or leave [0, num_tokens], or
- * whose slots do not fit its block table, sets KYRO_DEV_BAD_LENGTH and is
- * left out.  A stride is the number of elements from one row to the next
- * (0: dense), a multiple of 8, so the parts of one fused projection's rows
- * can be passed as they are. */
+ * Rows before chunk_starts[0] and from chunk_starts[B] on are padding: what
+ * they hold reaches no result, and what lies there in an output is left as it
+ * was.  A sequence whose chunk_starts entries decrease or leave [0,
+ * num_tokens], or whose slots do not fit its block table, sets
+ * KYRO_DEV_BAD_LENGTH and is left out; the others are served.  (Past a
+ * decrease two of them can claim a row: it is served as a row of either.)  A
+ * call without rows or sequences does nothing.  A stride is the number of
+ * elements from one row to the next (0: dense), a multiple of 8, so the parts
+ * of one fused projection's rows can be passed as they are. */
 typedef struct kyro_chunk_params {
   int32_t batch;              /* B                                              */
   int32_t num_tokens;         /* T rows in the packed tensors                   */

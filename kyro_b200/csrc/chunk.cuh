@@ -25,11 +25,7 @@ struct Seq {
   int bad;
 };
 
-__device__ __forceinline__ Seq seq_of(int b, const int32_t* __restrict__ starts,
-                                      const int64_t* __restrict__ context_lens, int T,
-                                      int max_slots) {
-  const int s0 = __ldg(&starts[b]), s1 = __ldg(&starts[b + 1]);
-  const int64_t ctx = __ldg(&context_lens[b]);
+__device__ __forceinline__ Seq seq_from(int s0, int s1, int64_t ctx, int T, int max_slots) {
   Seq s;
   s.start = s0;
   s.n = s1 - s0;
@@ -42,6 +38,13 @@ __device__ __forceinline__ Seq seq_of(int b, const int32_t* __restrict__ starts,
   if (s.bad) s.n = 0;
   s.ctx = (int)ctx;
   return s;
+}
+
+__device__ __forceinline__ Seq seq_of(int b, const int32_t* __restrict__ starts,
+                                      const int64_t* __restrict__ context_lens, int T,
+                                      int max_slots) {
+  return seq_from(__ldg(&starts[b]), __ldg(&starts[b + 1]), __ldg(&context_lens[b]), T,
+                  max_slots);
 }
 
 // ---------------------------------------------------------------- the walk

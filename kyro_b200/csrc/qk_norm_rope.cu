@@ -113,8 +113,43 @@ qk_norm_rope_kernel(const __grid_constant__ NormRopeArgs a, const uint16_t* __re
   Item cur, nxt;
   load(cur, threadIdx.x);
 
+  // The sequences that cannot be taken are flagged by one CTA; all see whether
+  // the starts are in order, which the search goes by.  Loaded here and looked
+  // at behind the search, from the last warp down, since a decode step's
+  // tokens are the first warps'.
+  const int b_first = kThreads - 1 - (int)threadIdx.x;
+  int first0 = 0, first1 = 0;
+  int64_t first_len = 0;
+  if (b_first < a.B) {
+    first0 = __ldg(&starts[b_first]);
+    first1 = __ldg(&starts[b_first + 1]);
+    if (blockIdx.x == 0) first_len = __ldg(&context_lens[b_first]);
+  }
+  // by one lane: where token t of sequence b goes (b -1 or a.B: it is padding)
+  auto put = [&](int tl, int t, int b) {
+    int64_t row = -1, pos = 0;
+    int ok = 0;
+    if (b >= 0 && b < a.B) {
+      const kyro::chunk::Seq s =
+          kyro::chunk::seq_of(b, starts, context_lens, a.T, a.max_blocks * a.bs);
+      const int j = t - s.start;
+      if (j >= 0 && j < s.n) {
+        ok = 1;
+        const int slot = s.ctx + j;
+        pos = positions ? positions[t] : slot;
+        const int64_t blk = block_table[(int64_t)b * a.max_blocks + slot / a.bs];
+        if (blk < 0 || blk >= a.num_blocks)
+          kyro::dev::flag(status, KYRO_DEV_BAD_BLOCK);
+        else
+          row = blk * a.hkv * a.bs + slot % a.bs;
+      }
+    }
+    sh_row[tl] = row;
+    sh_pos[tl] = pos;
+    sh_ok[tl] = ok;
+  };
   // the sequence of each token: the last b with starts[b] <= t, by two
-  // rounds of 32 lanes (B <= 1024; more rounds beyond)
+  // rounds of 32 lanes (B <= 1023; more rounds beyond)
   for (int tl = warp; tl < nt; tl += kThreads / 32) {
     const int t = t0 + tl;
     int lo = 0, n = a.B + 1;  // starts[lo .. lo + n) holds the answer's upper neighbour
@@ -131,32 +166,37 @@ qk_norm_rope_kernel(const __grid_constant__ NormRopeArgs a, const uint16_t* __re
       lo += first;
       n = min(step, n - first);
     }
-    if (lane == 0) {
-      int64_t row = -1, pos = 0;
-      int ok = 0;
-      if (lo >= 0 && lo < a.B) {
-        const kyro::chunk::Seq s =
-            kyro::chunk::seq_of(lo, starts, context_lens, a.T, a.max_blocks * a.bs);
-        const int j = t - s.start;
-        if (s.bad) {
-          kyro::dev::flag(status, KYRO_DEV_BAD_LENGTH);
-        } else if (j >= 0 && j < s.n) {
-          ok = 1;
-          const int slot = s.ctx + j;
-          pos = positions ? positions[t] : slot;
-          const int64_t blk = block_table[(int64_t)lo * a.max_blocks + slot / a.bs];
-          if (blk < 0 || blk >= a.num_blocks)
-            kyro::dev::flag(status, KYRO_DEV_BAD_BLOCK);
-          else
-            row = blk * a.hkv * a.bs + slot % a.bs;
-        }
-      }
-      sh_row[tl] = row;
-      sh_pos[tl] = pos;
-      sh_ok[tl] = ok;
-    }
+    if (lane == 0) put(tl, t, lo);
   }
-  __syncthreads();
+  bool disorder = first0 > first1;
+  bool bad = blockIdx.x == 0 &&
+             kyro::chunk::seq_from(first0, first1, first_len, a.T, a.max_blocks * a.bs).bad;
+  for (int b = b_first + kThreads; b < a.B; b += kThreads) {
+    disorder |= __ldg(&starts[b]) > __ldg(&starts[b + 1]);
+    bad |= blockIdx.x == 0 &&
+           kyro::chunk::seq_of(b, starts, context_lens, a.T, a.max_blocks * a.bs).bad;
+  }
+  if (bad) kyro::dev::flag(status, KYRO_DEV_BAD_LENGTH);
+  if (__syncthreads_or(disorder)) {
+    // a start that decreases leads the search astray: the last of the
+    // sequences that hold the token, among those that can be taken
+    for (int tl = warp; tl < nt; tl += kThreads / 32) {
+      const int t = t0 + tl;
+      int last = -1;
+      for (int b0 = 0; b0 < a.B; b0 += 32) {
+        bool holds = false;
+        if (b0 + lane < a.B) {
+          const kyro::chunk::Seq s =
+              kyro::chunk::seq_of(b0 + lane, starts, context_lens, a.T, a.max_blocks * a.bs);
+          holds = t >= s.start && t - s.start < s.n;
+        }
+        const uint32_t m = __ballot_sync(0xffffffffu, holds);
+        if (m) last = b0 + 31 - __clz(m);
+      }
+      if (lane == 0) put(tl, t, last);
+    }
+    __syncthreads();
+  }
   for (int i = threadIdx.x; i < nt * half; i += kThreads) {
     const int tl = i / half, f = i - tl * half;
     // reduced by a multiple of 2 pi, whose two parts hold 106 bits

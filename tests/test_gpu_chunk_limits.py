@@ -47,3 +47,63 @@ def test_scores_of_a_very_long_context(ctx, heads, ctx_len):
     for i in range(16):
         assert ((got[i::16].double() - want[i]).abs() <= 2.0 ** -11 * want[i]).all(), i
     assert (scores[0, 0, ctx_len + 1:] == 0).all()
+
+
+def _bad_starts(kind, B, n):
+    rng = np.random.default_rng(7)
+    s = np.arange(B + 1) * n
+    if kind == "scattered":  # a few entries that go back into the sequence before
+        s[np.arange(2, B - 8, 9) + rng.integers(0, 7)] -= n + 1
+    elif kind == "reversed":
+        s = s[::-1].copy()
+    elif kind == "past the end":
+        s[-1] += 1
+    elif kind == "below zero":
+        s[0] = -1
+    elif kind == "starts late":
+        s[0] = s[1] + 1
+    return [int(i) for i in s]
+
+
+@pytest.mark.parametrize("starts", [[0, 4, -1, 12], [0, 12, 13, 13], [0, 4, 3, 12], [0, 4, 8, 13],
+                                    [-1, 4, 8, 12], [5, 4, 8, 12], [0, 8, 4, 12], [12, 8, 4, 0],
+                                    [0, 0, 12, 12], [0, 4, 13, 12]] +
+                         [_bad_starts(k, 100, 3) for k in (
+                             "scattered", "reversed", "past the end", "below zero",
+                             "starts late")] + [_bad_starts("scattered", 1500, 2)])
+def test_norm_rope_write_beside_bad_starts(ctx, starts):
+    """Sequences whose starts cannot be are flagged and left out, the others
+    served, whatever order the starts are in."""
+    from kyro_b200._lib import DEV_BAD_LENGTH
+    from kyro_b200.verify import qk_norm_rope_kv_write
+    B = len(starts) - 1
+    T = 12 if B == 3 else B * (3 if B == 100 else 2)
+    lens = [20 + b % 5 for b in range(B)]
+    # (each sequence has room for all rows)
+    x = R.Batch(ctx.device, [12] * B, lens, 2, 1, 64, seed=1)
+    q, k, v = (torch.randn(T, h, 64, device=ctx.device).bfloat16() for h in (2, 1, 1))
+    out, kc, vc = torch.full_like(q, 7.0), x.k_cache.clone(), x.v_cache.clone()
+    st = torch.tensor(starts, dtype=torch.int32, device=ctx.device)
+    qk_norm_rope_kv_write(ctx, q, k, v, st, x.block_table, x.context_lens, kc, vc, 16, q_out=out)
+    width = x.block_table.shape[1] * 16
+    good = [b for b in range(B) if 0 <= starts[b] <= starts[b + 1] <= T
+            and (starts[b] == starts[b + 1] or lens[b] + starts[b + 1] - starts[b] <= width)]
+    assert ctx.device_status() == (0 if len(good) == B else DEV_BAD_LENGTH)
+    for t in range(T):
+        held = [b for b in good if starts[b] <= t < starts[b + 1]]
+        if not held:
+            assert (out[t] == 7.0).all()
+            continue
+        fits = 0
+        for b in held:
+            slot = lens[b] + t - starts[b]
+            at = torch.tensor([slot], device=ctx.device)
+            ref, mag = R.norm_rope(q[t:t + 1], None, at, 0.0, 10000.0)
+            rk, mk = R.norm_rope(k[t:t + 1], None, at, 0.0, 10000.0)
+            blk, off = int(x.host_table[b, slot // 16]), slot % 16
+            fits += int(((out[t].double() - ref[0]).abs()
+                         <= U * ref[0].abs() + 2.0 ** -20 * mag[0]).all() and
+                        ((kc[blk, :, off].double() - rk[0]).abs()
+                         <= U * rk[0].abs() + 2.0 ** -20 * mk[0]).all() and
+                        _same(vc[blk, :, off], v[t]))
+        assert fits >= 1, (t, held)
