@@ -27,15 +27,10 @@ struct Seq {
 
 __device__ __forceinline__ Seq seq_from(int s0, int s1, int64_t ctx, int T, int max_slots) {
   Seq s;
+  const int n = chunk_rows(s0, s1, ctx, T, max_slots);
   s.start = s0;
-  s.n = s1 - s0;
-  s.bad = 0;
-  if (s0 < 0 || s1 < s0 || s1 > T) {
-    s.bad = 1;
-  } else if (s.n > 0 && (ctx < 0 || ctx + s.n > max_slots)) {
-    s.bad = 1;
-  }
-  if (s.bad) s.n = 0;
+  s.bad = n < 0;
+  s.n = n < 0 ? 0 : n;
   s.ctx = (int)ctx;
   return s;
 }

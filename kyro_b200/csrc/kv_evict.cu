@@ -51,7 +51,7 @@ struct LayerPtrs {
 // reserved ones too) fit the table and the scores
 __device__ __forceinline__ bool over(const EvictArgs& a, int64_t len) { return len > a.budget; }
 __device__ __forceinline__ bool fits(const EvictArgs& a, int64_t len) {
-  return len + a.reserved <= (int64_t)a.max_blocks * a.bs && len <= a.score_slots;
+  return kyro::chunk::evict_fits(len, a.reserved, (int64_t)a.max_blocks * a.bs, a.score_slots);
 }
 __device__ __forceinline__ int clamp_top(int t, int num_blocks) {
   return t < 0 ? 0 : t > num_blocks ? num_blocks : t;

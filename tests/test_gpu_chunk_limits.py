@@ -107,3 +107,43 @@ def test_norm_rope_write_beside_bad_starts(ctx, starts):
                          <= U * rk[0].abs() + 2.0 ** -20 * mk[0]).all() and
                         _same(vc[blk, :, off], v[t]))
         assert fits >= 1, (t, held)
+
+
+@pytest.mark.parametrize("length", [(1 << 63) - 1, (1 << 63) - 4, 1 << 62, (1 << 32) + 20, 1 << 31,
+                                    -1, -(1 << 31) + 20, -(1 << 63)])
+def test_lengths_that_no_table_holds(ctx, length):
+    """Flagged and left out, however the new rows are added to them."""
+    from kyro_b200._lib import DEV_BAD_LENGTH
+    from kyro_b200.verify import chunk_attention, kv_evict, kv_scores_add, qk_norm_rope_kv_write
+    x = R.Batch(ctx.device, [4, 4, 4], [20, 20, 20], 4, 2, 64, seed=1)
+    want, lse = torch.empty_like(x.q), torch.zeros(x.T, x.hq, device=ctx.device)
+    chunk_attention(ctx, x.q, x.k_cache, x.v_cache, x.chunk_starts, x.block_table, x.context_lens,
+                    out=want, lse=lse)
+    lens = x.context_lens.clone()
+    lens[1] = length
+    out, ls = torch.full_like(x.q, 7.0), torch.full_like(lse, 7.0)
+    chunk_attention(ctx, x.q, x.k_cache, x.v_cache, x.chunk_starts, x.block_table, lens, out=out,
+                    lse=ls)
+    assert ctx.device_status() == DEV_BAD_LENGTH
+    assert (out[4:8] == 7.0).all() and (ls[4:8] == 7.0).all()
+    assert _same(out[:4], want[:4]) and _same(out[8:], want[8:])
+    s = torch.full((3, 2, 200), 3.0, device=ctx.device)
+    kv_scores_add(ctx, x.q, x.k_cache, lse, x.chunk_starts, x.block_table, lens, s)
+    assert ctx.device_status() == DEV_BAD_LENGTH
+    assert (s[1] == 3.0).all() and (s[0, :, :20] > 3.0).all() and (s[2, :, :20] > 3.0).all()
+    kc, vc = x.k_cache.clone(), x.v_cache.clone()
+    qk_norm_rope_kv_write(ctx, x.q, x.k_new, x.v_new, x.chunk_starts, x.block_table, lens, kc, vc,
+                          16, q_out=out.fill_(7.0))
+    assert ctx.device_status() == DEV_BAD_LENGTH and (out[4:8] == 7.0).all()
+    blk, off = x.where(1, np.arange(24))
+    assert _same(kc[blk, :, off], x.k_cache[blk, :, off])
+    assert not (out[:4] == 7.0).all() and not (out[8:] == 7.0).all()
+    free = torch.arange(x.nb, dtype=torch.int32, device=ctx.device)
+    refs = torch.ones(x.nb, dtype=torch.int32, device=ctx.device)
+    kept = torch.empty(1, 3, 2, 8, dtype=torch.int32, device=ctx.device)
+    table, top = x.block_table.clone(), torch.zeros(1, dtype=torch.int32, device=ctx.device)
+    gone = kv_evict(ctx, 8, 1, 2, [s], [kc], [vc], table, lens, free, top, refs, 16,
+                    num_reserved=5, kept=kept)
+    assert gone.tolist() == [-1, -1 if length > 8 else 0, -1]  # (no free blocks)
+    assert ctx.device_status() == (DEV_BAD_LENGTH if length > 8 else 0)
+    assert torch.equal(table, x.block_table) and int(lens[1]) == length and (kept == -1).all()
