@@ -609,6 +609,19 @@ def _rows_arg(t: torch.Tensor, name: str, device, shape=None) -> tuple:
     return t.data_ptr(), got, st
 
 
+def _scratch(ctx: Context, workspace: Optional[torch.Tensor], need: int) -> tuple:
+    """The address and bytes of the caller's workspace, or of the context's."""
+    if workspace is None:
+        workspace = ctx.workspace(need)
+    elif not isinstance(workspace, torch.Tensor):
+        raise TypeError("workspace must be a torch.Tensor")
+    elif workspace.device != ctx.device:
+        raise ValueError(f"workspace must be on {ctx.device}, got {workspace.device}")
+    elif not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
 def _chunk_args(ctx: Context, chunk_starts, block_table, context_lens) -> tuple:
     """The addresses of a batch of chunks, its size and its table's width."""
     dev = ctx.device
@@ -728,10 +741,9 @@ def chunk_attention(ctx: Context, q: torch.Tensor, k_cache: torch.Tensor, v_cach
     p = ChunkParams(B, T, hq, hkv, d, bs, width, nb, scale or 0.0, qs, 0, 0, os)
     L = _lib.load()
     need = L.kyro_chunk_attention_workspace_size(p)
-    ws = workspace if workspace is not None else ctx.workspace(need)
+    wp, bytes_ = _scratch(ctx, workspace, need)
     ctx.bind_stream()
-    check(L.kyro_chunk_attention(ctx.handle, p, qp, kp, vp, sp, bp, lp, op, ep, ws.data_ptr(),
-                                 ws.numel()))
+    check(L.kyro_chunk_attention(ctx.handle, p, qp, kp, vp, sp, bp, lp, op, ep, wp, bytes_))
     return out
 
 
@@ -773,10 +785,10 @@ def kv_scores_add(ctx: Context, q: torch.Tensor, k_cache: torch.Tensor, lse: tor
     p = ChunkParams(B, T, hq, hkv, d, bs, width, nb, scale or 0.0, qs, 0, 0, 0)
     L = _lib.load()
     need = L.kyro_kv_scores_add_workspace_size(p)
-    ws = workspace if workspace is not None else ctx.workspace(need)
+    wp, bytes_ = _scratch(ctx, workspace, need)
     ctx.bind_stream()
     check(L.kyro_kv_scores_add(ctx.handle, p, qp, kp, ep, sp, bp, lp, shape[2], scp, op,
-                               ws.data_ptr(), ws.numel()))
+                               wp, bytes_))
     return out
 
 
@@ -842,11 +854,11 @@ def kv_evict(ctx: Context, budget: int, num_sink: int, num_recent: int,
                     num_reserved, sshape[2])
     L = _lib.load()
     need = L.kyro_kv_evict_workspace_size(p)
-    ws = workspace if workspace is not None else ctx.workspace(need)
+    wp, bytes_ = _scratch(ctx, workspace, need)
     pointers = C.c_void_p * nl
     ctx.bind_stream()
     check(L.kyro_kv_evict(ctx.handle, p, pointers(*scp), pointers(*kp), pointers(*vp), bp, lp, fp,
-                          free_top.data_ptr(), rp, ep, tp, ws.data_ptr(), ws.numel()))
+                          free_top.data_ptr(), rp, ep, tp, wp, bytes_))
     return evicted
 
 
