@@ -7,6 +7,7 @@ missing, importing the package's operators raises.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -211,19 +212,23 @@ _calls = None
 
 def calls():
     """The extension module with the chunk operators' Python calls, bound to
-    the library that load() gave (once).  Raises if it has not been built."""
+    the library that load() gave (once).  Raises if it has not been built for
+    this Python and this torch."""
     global _calls
     if _calls is None:
-        if not os.path.exists(os.path.join(_HERE, "_pycall.so")):
-            raise ImportError("kyro_b200/_pycall.so is missing: build it with "
-                              "`python -m kyro_b200.build`")
-        import torch  # noqa: F401  (the module's own libraries)
-        from . import _pycall
+        import torch
+        from .build import pycall_path
+        path = pycall_path(torch.__version__)
+        if not os.path.exists(path):
+            raise ImportError(f"{path} is missing: build it with `python -m kyro_b200.build`")
+        spec = importlib.util.spec_from_file_location(__package__ + "._pycall", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
         L = load()
-        _pycall.bind(*(C.cast(getattr(L, name), C.c_void_p).value for name in (
+        module.bind(*(C.cast(getattr(L, name), C.c_void_p).value for name in (
             "kyro_qk_norm_rope_kv_write", "kyro_chunk_attention",
             "kyro_chunk_attention_workspace_size", "kyro_kv_scores_add",
             "kyro_kv_scores_add_workspace_size", "kyro_kv_evict",
             "kyro_kv_evict_workspace_size")))
-        _calls = _pycall
+        _calls = module
     return _calls

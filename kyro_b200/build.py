@@ -5,8 +5,9 @@ Usage: python -m kyro_b200.build [--force] [--verbose]
 Each translation unit compiles to an object under kyro_b200/_build/, then
 nvcc links them into one shared library with the CUDA runtime linked
 statically (the library exports only the C ABI of include/kyro_spec.h).
-csrc/pycall.cpp, the Python calls of the chunk operators, becomes the
-extension module kyro_b200/_pycall.so beside it.
+csrc/pycall.cpp, the Python calls of the chunk operators, becomes an extension
+module beside it, for the torch and the Python that it is built with: it reads
+torch's tensors in place, so its file is named after both (pycall_path).
 sampler.cu is compiled with --fmad=false: its arithmetic must round exactly
 like the CPU restatement it is checked against.
 """
@@ -15,6 +16,7 @@ from __future__ import annotations
 import argparse
 import importlib.util
 import os
+import runpy
 import shutil
 import subprocess
 import sys
@@ -25,7 +27,6 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libkyro_spec.so")
-PYCALL = os.path.join(HERE, "_pycall.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-ffp-contract=off",
@@ -80,19 +81,25 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return LIB
 
 
+def pycall_path(torch_version: str) -> str:
+    """The extension module for this Python and a version of torch."""
+    return os.path.join(HERE, f"_pycall-torch{torch_version}"
+                        f"{sysconfig.get_config_var('EXT_SUFFIX')}")
+
+
 def _build_pycall(force: bool, verbose: bool):
     src = os.path.join(CSRC, "pycall.cpp")
-    if not (force or _stale(PYCALL, [src, os.path.join(ROOT, "include", "kyro_spec.h"),
-                                     __file__])):
-        return
     torch = os.path.dirname(importlib.util.find_spec("torch").origin)
+    out = pycall_path(runpy.run_path(os.path.join(torch, "version.py"))["__version__"])
+    if not (force or _stale(out, [src, os.path.join(ROOT, "include", "kyro_spec.h"), __file__])):
+        return
     cuda = os.path.dirname(os.path.dirname(nvcc()))
     inc = [os.path.join(torch, "include"),
            os.path.join(torch, "include", "torch", "csrc", "api", "include"),
            sysconfig.get_paths()["include"], os.path.join(cuda, "include"),
            os.path.join(ROOT, "include")]
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
-           *["-I" + i for i in inc], src, "-o", PYCALL, "-L" + os.path.join(torch, "lib"),
+           *["-I" + i for i in inc], src, "-o", out, "-L" + os.path.join(torch, "lib"),
            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"]
     if verbose:
         print(" ".join(cmd), flush=True)
