@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import importlib.util
 import os
+import warnings
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libkyro_spec.so")
@@ -212,18 +213,22 @@ _calls = None
 
 def calls():
     """The extension module with the chunk operators' Python calls, bound to
-    the library that load() gave (once).  Raises if it has not been built for
-    this Python and this torch."""
+    the library that load() gave (once).  None, with a warning, where it has
+    not been built for this Python and this torch: the operators then make
+    their calls through ctypes, at 10 to 15 us more each."""
     global _calls
     if _calls is None:
         import torch
         from .build import pycall_path
         path = pycall_path(torch.__version__)
-        if not os.path.exists(path):
-            raise ImportError(f"{path} is missing: build it with `python -m kyro_b200.build`")
         spec = importlib.util.spec_from_file_location(__package__ + "._pycall", path)
-        module = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(module)
+        try:
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except ImportError as e:
+            warnings.warn(f"no extension module for this torch and Python ({e}); "
+                          "`python -m kyro_b200.build` makes it", RuntimeWarning, stacklevel=2)
+            return None
         L = load()
         module.bind(*(C.cast(getattr(L, name), C.c_void_p).value for name in (
             "kyro_qk_norm_rope_kv_write", "kyro_chunk_attention",

@@ -8,6 +8,8 @@ statically (the library exports only the C ABI of include/kyro_spec.h).
 csrc/pycall.cpp, the Python calls of the chunk operators, becomes an extension
 module beside it, for the torch and the Python that it is built with: it reads
 torch's tensors in place, so its file is named after both (pycall_path).
+Without torch's or Python's headers, or a host C++ compiler, the library is
+built all the same.
 sampler.cu is compiled with --fmad=false: its arithmetic must round exactly
 like the CPU restatement it is checked against.
 """
@@ -89,7 +91,10 @@ def pycall_path(torch_version: str) -> str:
 
 def _build_pycall(force: bool, verbose: bool):
     src = os.path.join(CSRC, "pycall.cpp")
-    torch = os.path.dirname(importlib.util.find_spec("torch").origin)
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        return _no_pycall("torch is not installed")
+    torch = os.path.dirname(spec.origin)
     out = pycall_path(runpy.run_path(os.path.join(torch, "version.py"))["__version__"])
     if not (force or _stale(out, [src, os.path.join(ROOT, "include", "kyro_spec.h"), __file__])):
         return
@@ -103,7 +108,18 @@ def _build_pycall(force: bool, verbose: bool):
            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"]
     if verbose:
         print(" ".join(cmd), flush=True)
-    subprocess.run(cmd, check=True)
+    if os.path.exists(out):
+        os.remove(out)
+    try:
+        subprocess.run(cmd, check=True)
+    except (OSError, subprocess.CalledProcessError) as e:
+        _no_pycall(str(e))
+
+
+def _no_pycall(why: str):
+    """The library is complete without the module; its calls are what it is for."""
+    print(f"kyro_b200: no extension module, Python calls go through ctypes ({why})",
+          file=sys.stderr, flush=True)
 
 
 def main(argv=None):

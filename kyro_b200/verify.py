@@ -658,7 +658,7 @@ def qk_norm_rope_kv_write(ctx: Context, q: torch.Tensor, k_new: torch.Tensor,
     (chunk_starts int32 [B + 1]), the queries into q_out (default a new
     tensor; q itself is allowed).  Rows of q, k_new, v_new and q_out may lie
     apart.  positions int64 [T]: rotary positions (default the slots)."""
-    if type(ctx) is Context:
+    if type(ctx) is Context and ctx._calls is not None:
         ctx.bind_stream()
         r = ctx._calls.qk_norm_rope_kv_write(
             ctx._h.value, ctx.index, q, k_new, v_new, chunk_starts, block_table, context_lens,
@@ -713,7 +713,7 @@ def chunk_attention(ctx: Context, q: torch.Tensor, k_cache: torch.Tensor, v_cach
     [T, Hq, D] and fills lse fp32 [T, Hq] when given.  Rows of q and out may
     lie apart.  A call captured into a graph should be given its own
     workspace (uint8, kyro_chunk_attention_workspace_size bytes)."""
-    if type(ctx) is Context:
+    if type(ctx) is Context and ctx._calls is not None:
         ctx.bind_stream()
         r = ctx._calls.chunk_attention(
             ctx._h.value, ctx.index, q, k_cache, v_cache, chunk_starts, block_table, context_lens,
@@ -756,7 +756,7 @@ def kv_scores_add(ctx: Context, q: torch.Tensor, k_cache: torch.Tensor, lse: tor
     the chunks' rows q bf16 [T, Hq, D] (lse fp32 [T, Hq] from chunk_attention
     on the same rows), added to scores fp32 [B, Hkv, slots].  In place unless
     out is given.  Returns the scores."""
-    if type(ctx) is Context:
+    if type(ctx) is Context and ctx._calls is not None:
         ctx.bind_stream()
         r = ctx._calls.kv_scores_add(
             ctx._h.value, ctx.index, q, k_cache, lse, chunk_starts, block_table, context_lens,
@@ -804,7 +804,7 @@ def kv_evict(ctx: Context, budget: int, num_sink: int, num_recent: int,
     up into fresh blocks.  Returns evicted int32 [B] (slots dropped; 0 within
     the budget; -1 over it but left as it was) and fills kept int32 [layers,
     B, Hkv, budget] with the old slots when given."""
-    if type(ctx) is Context:
+    if type(ctx) is Context and ctx._calls is not None:
         ctx.bind_stream()
         r = ctx._calls.kv_evict(
             ctx._h.value, ctx.index, budget, num_sink, num_recent, scores, k_caches, v_caches,
