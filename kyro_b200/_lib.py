@@ -231,7 +231,7 @@ def calls():
             return None
         L = load()
         module.bind(*(C.cast(getattr(L, name), C.c_void_p).value for name in (
-            "kyro_qk_norm_rope_kv_write", "kyro_chunk_attention",
+            "kyro_ctx_set_stream", "kyro_qk_norm_rope_kv_write", "kyro_chunk_attention",
             "kyro_chunk_attention_workspace_size", "kyro_kv_scores_add",
             "kyro_kv_scores_add_workspace_size", "kyro_kv_evict",
             "kyro_kv_evict_workspace_size")))

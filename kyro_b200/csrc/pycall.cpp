@@ -19,6 +19,7 @@
 namespace {
 
 struct {
+  decltype(&kyro_ctx_set_stream) set_stream;
   decltype(&kyro_qk_norm_rope_kv_write) rope;
   decltype(&kyro_chunk_attention) attention;
   decltype(&kyro_chunk_attention_workspace_size) attention_workspace;
@@ -332,27 +333,44 @@ PyObject* entry(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
 }
 
-// bind: the addresses of the library's seven entry points, in lib's order
-PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 7) {
+// (ctx, stream): the status of kyro_ctx_set_stream
+PyObject* set_stream(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 2) {
     PyErr_SetString(PyExc_TypeError, "wrong number of arguments");
     return nullptr;
   }
-  void* f[7];
-  for (int i = 0; i < 7; ++i) f[i] = PyLong_AsVoidPtr(a[i]);
-  if (PyErr_Occurred()) return nullptr;
-  lib.rope = (decltype(lib.rope))f[0];
-  lib.attention = (decltype(lib.attention))f[1];
-  lib.attention_workspace = (decltype(lib.attention_workspace))f[2];
-  lib.scores = (decltype(lib.scores))f[3];
-  lib.scores_workspace = (decltype(lib.scores_workspace))f[4];
-  lib.evict = (decltype(lib.evict))f[5];
-  lib.evict_workspace = (decltype(lib.evict_workspace))f[6];
+  kyro_ctx* ctx = (kyro_ctx*)PyLong_AsVoidPtr(a[0]);
+  void* stream = PyErr_Occurred() ? nullptr : PyLong_AsVoidPtr(a[1]);
+  if (PyErr_Occurred() || !lib.set_stream) return unsure();
+  return PyLong_FromLong(lib.set_stream(ctx, stream));
+}
+
+// bind: the addresses of the library's entry points, in lib's order
+PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  constexpr int kEntries = 8;
+  if (n != kEntries) {
+    PyErr_SetString(PyExc_TypeError, "wrong number of arguments");
+    return nullptr;
+  }
+  void* f[kEntries];
+  for (int i = 0; i < kEntries; ++i) {
+    f[i] = PyLong_AsVoidPtr(a[i]);
+    if (PyErr_Occurred()) return nullptr;
+  }
+  lib.set_stream = (decltype(lib.set_stream))f[0];
+  lib.rope = (decltype(lib.rope))f[1];
+  lib.attention = (decltype(lib.attention))f[2];
+  lib.attention_workspace = (decltype(lib.attention_workspace))f[3];
+  lib.scores = (decltype(lib.scores))f[4];
+  lib.scores_workspace = (decltype(lib.scores_workspace))f[5];
+  lib.evict = (decltype(lib.evict))f[6];
+  lib.evict_workspace = (decltype(lib.evict_workspace))f[7];
   Py_RETURN_NONE;
 }
 
 PyMethodDef methods[] = {
     {"bind", (PyCFunction)(void (*)(void))bind, METH_FASTCALL, nullptr},
+    {"set_stream", (PyCFunction)(void (*)(void))set_stream, METH_FASTCALL, nullptr},
     {"qk_norm_rope_kv_write", (PyCFunction)(void (*)(void))entry<rope_impl, 17>, METH_FASTCALL,
      nullptr},
     {"chunk_attention", (PyCFunction)(void (*)(void))entry<attention_impl, 12>, METH_FASTCALL,

@@ -60,7 +60,6 @@ class Context:
             stream = torch.cuda.current_stream(device).cuda_stream
             check(L.kyro_ctx_create(device, C.c_void_p(stream), C.byref(h)))
         self._h = h
-        self._stream = stream
         self._ws: Optional[torch.Tensor] = None
         self._calls = _lib.calls()
 
@@ -69,10 +68,16 @@ class Context:
         return self._h
 
     def bind_stream(self):
+        """Torch's current stream is the context's from here on, whichever it
+        had (kyro_ctx_set_stream on the handle may have changed it)."""
         stream = _raw_stream(self.index)
-        if stream != self._stream:
-            check(_lib.load().kyro_ctx_set_stream(self._h, C.c_void_p(stream)))
-            self._stream = stream
+        status = None
+        if self._calls is not None:
+            status = self._calls.set_stream(self._h.value, stream)
+        if status is None:
+            status = _lib.load().kyro_ctx_set_stream(self._h, C.c_void_p(stream))
+        if status:
+            check(status)
 
     def workspace(self, nbytes: int) -> torch.Tensor:
         """A caller-owned scratch buffer of at least nbytes (grown on demand)."""
