@@ -353,7 +353,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ,
         if (j + 1 < ntiles) fetch_ids(j + 1);
         bool stop = false;
         for (int n = 2 * j; n < 2 * j + 2; ++n) {
-          if (n >= kSlots && !wait_bar(slot_empty(item_slot(n)), item_parity(n - kSlots), err, status)) {
+          if (n >= kSlots && !wait_bar<false>(slot_empty(item_slot(n)), item_parity(n - kSlots), err, status)) {
             stop = true;
             break;
           }
@@ -389,9 +389,9 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ,
       auto o_mma = [&](int h, int j) -> bool {
         const uint32_t vs = item_addr(2 * j + 1);
         for (int half = 0; half < 2; ++half) {
-          if (!wait_bar(p_full(h, half), j & 1, err, status)) return false;
+          if (!wait_bar<false>(p_full(h, half), j & 1, err, status)) return false;
           if (half == 0 && h == 0 &&
-              !wait_bar(slot_full(item_slot(2 * j + 1)), item_parity(2 * j + 1), err, status))
+              !wait_bar<false>(slot_full(item_slot(2 * j + 1)), item_parity(2 * j + 1), err, status))
             return false;
           tc_fence_after();
 #pragma unroll
@@ -405,7 +405,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ,
         if (h == ntq - 1) umma2_commit_both(slot_empty(item_slot(2 * j + 1)));  // V_j no longer read
         return true;
       };
-      bool ok = wait_bar(q_full(), 0, err, status) && wait_bar(slot_full(0), 0, err, status);
+      bool ok = wait_bar<false>(q_full(), 0, err, status) && wait_bar<false>(slot_full(0), 0, err, status);
       if (ok) {
         tc_fence_after();
         for (int h = 0; h < ntq; ++h) s_mma(h, 0);
@@ -425,7 +425,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ,
           if (more) {
             if (h == 0) {
               const int nk = 2 * (j + 1);
-              if (!wait_bar(slot_full(item_slot(nk)), item_parity(nk), err, status)) {
+              if (!wait_bar<false>(slot_full(item_slot(nk)), item_parity(nk), err, status)) {
                 ok = false;
                 break;
               }
@@ -438,7 +438,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ,
       // every MMA issued above is complete before either CTA frees TMEM
       umma2_commit_both(mma_done);
     }
-    if (lane == 0) wait_bar(mma_done, 0, err, status);
+    if (lane == 0) wait_bar<false>(mma_done, 0, err, status);
     __syncwarp();
   } else if (warp < 8 && warp / 4 < ntq) {
     // ------------------------------------------------ softmax of tile h, one row per thread
@@ -472,7 +472,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ,
     float m_used = -INFINITY, l = 0.0f;
     bool ok = true;
     for (int j = 0; j < ntiles; ++j) {
-      if (!wait_bar(s_full(h), j & 1, err, status)) {
+      if (!wait_bar<false>(s_full(h), j & 1, err, status)) {
         ok = false;
         break;
       }
@@ -505,7 +505,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ,
       if (__any_sync(0xffffffffu, need)) {
         // S_h of tile j was issued after O_h of tile j-1, so O_h is final
         // for tile j-1 by now; the wait only confirms it
-        if (!wait_bar(o_done(h), (j - 1) & 1, err, status)) {
+        if (!wait_bar<false>(o_done(h), (j - 1) & 1, err, status)) {
           ok = false;
           break;
         }
@@ -548,7 +548,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ,
         mbar_arrive_cluster(half == 0 ? pf0 : pf1);
       }
     }
-    if (ok && real && ntiles > 0 && wait_bar(o_done(h), (ntiles - 1) & 1, err, status)) {
+    if (ok && real && ntiles > 0 && wait_bar<false>(o_done(h), (ntiles - 1) & 1, err, status)) {
       tc_fence_after();
       const float inv = l > 0.0f ? 1.0f / l : 0.0f;
       __nv_bfloat16* orow =
