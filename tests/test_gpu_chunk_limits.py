@@ -147,3 +147,62 @@ def test_lengths_that_no_table_holds(ctx, length):
     assert gone.tolist() == [-1, -1 if length > 8 else 0, -1]  # (no free blocks)
     assert ctx.device_status() == (DEV_BAD_LENGTH if length > 8 else 0)
     assert torch.equal(table, x.block_table) and int(lens[1]) == length and (kept == -1).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("base,gap", [(0, 8), (0, 16), (8, 16), (8, 24), (16, 48)])
+@pytest.mark.parametrize("chunks,ctxs", [([300, 1, 70], [0, 40, 17]), ([3], [9000]),
+                                         ([1] * 30, list(range(0, 30 * 90, 90)))])
+def test_attention_into_rows_that_lie_apart(ctx, d, base, gap, chunks, ctxs):
+    """An output that is part of wider rows, on 16 and on 32 bytes, from whole
+    items and from joined ones: the same bits as a dense one, and nothing
+    beside them."""
+    from kyro_b200.verify import chunk_attention
+    x = R.Batch(ctx.device, chunks, ctxs, 8, 2, d, seed=d + gap, front=2, back=1)
+    row = x.hq * d
+
+    def call(out):
+        lse = torch.full((x.T, x.hq), 7.0, device=ctx.device)
+        chunk_attention(ctx, x.q, x.k_cache, x.v_cache, x.chunk_starts, x.block_table,
+                        x.context_lens, out=out, lse=lse)
+        return lse
+
+    want = torch.full((x.T, x.hq, d), 7.0, dtype=torch.bfloat16, device=ctx.device)
+    want_lse = call(want)
+    ref, _, mag = R.attention(x)
+    err = (want.double() - ref).abs()[2:-1]
+    assert (err <= (U * ref.abs() + (U + 2.0 ** -11) * mag)[2:-1]).all()
+    whole = torch.full((x.T, row + gap), 7.0, dtype=torch.bfloat16, device=ctx.device)
+    # (a view that begins `base` elements into its rows)
+    out = whole[:, base:base + row].unflatten(1, (x.hq, d))
+    lse = call(out)
+    assert ctx.device_status() == 0
+    assert _same(out, want) and _same(lse, want_lse)
+    assert (whole[:, :base] == 7.0).all() and (whole[:, base + row:] == 7.0).all()
+
+
+@pytest.mark.parametrize("gap", [8, 32])
+def test_norm_rope_into_rows_that_lie_apart(ctx, gap):
+    from kyro_b200.verify import qk_norm_rope_kv_write
+    x = R.Batch(ctx.device, [70, 1, 9], [3, 40, 0], 6, 2, 128, seed=gap, gap=gap, front=1, back=2)
+    args = (x.k_new, x.v_new, x.chunk_starts, x.block_table, x.context_lens, x.k_cache, x.v_cache,
+            16)
+    want = qk_norm_rope_kv_write(ctx, x.q, *args, q_out=torch.full(
+        (x.T, 6, 128), 7.0, dtype=torch.bfloat16, device=ctx.device))
+    whole = torch.full((x.T, 6 * 128 + gap), 7.0, dtype=torch.bfloat16, device=ctx.device)
+    out = whole[:, 8:8 + 6 * 128].unflatten(1, (6, 128))
+    qk_norm_rope_kv_write(ctx, x.q, *args, q_out=out)
+    assert ctx.device_status() == 0 and _same(out, want)
+    assert (whole[:, :8] == 7.0).all() and (whole[:, 8 + 6 * 128:] == 7.0).all()
+
+
+@pytest.mark.parametrize("width,sequences", [(32768, 60), (49152 - 64, 20), (131072, 30)])
+def test_evict_short_rows_of_a_wide_table(ctx, width, sequences):
+    """Tables far wider than their sequences, as a server's are, and many
+    sequences: selections that hold their rows on chip and ones that do not."""
+    import test_gpu_evict as E
+    lens = [(37 * i) % 700 + 1 for i in range(sequences)]
+    st, s, k, v = E._state(ctx.device, lens, 2, 8, 1, 16, 211, 3, seed=sequences,
+                           width_extra=width // 16)
+    ev, flags = E._run(ctx, st, s, k, v, 211, 3, 50, 3, 16)
+    assert flags == 0 and all((e > 0) == (n > 211) for e, n in zip(ev, lens))
