@@ -395,6 +395,9 @@ int kyro_rope_kv_write(kyro_ctx* ctx, const kyro_kv_params* p, int32_t num_new,
  * num_tokens], or whose slots do not fit its block table, sets
  * KYRO_DEV_BAD_LENGTH and is left out; the others are served.  (Past a
  * decrease two of them can claim a row: it is served as a row of either.)  A
+ * block id outside [0, num_blocks) sets KYRO_DEV_BAD_BLOCK: new rows that
+ * belong there are not stored, and the attention and the scores of that
+ * sequence are formed with block 0 in its place, which says nothing.  A
  * call without rows or sequences does nothing.  A stride is the number of
  * elements from one row to the next (0: dense), a multiple of 8, so the parts
  * of one fused projection's rows can be passed as they are. */

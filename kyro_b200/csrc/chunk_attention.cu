@@ -43,10 +43,10 @@
 // at D = 128 (1024 at D = 64) and 2048 of exponentials on the special-function
 // unit, and it takes 3500 to 3700; an item costs 5400 beside its steps (2000
 // of them the stores of its rows), a call 7 us beside its items.  4096 rows
-// over 16384 slots, 64 heads of 128: 1.65 to 1.88 ms, 1.02 to 1.16 PFLOP/s as
-// the clock goes under the power limit; 12 prompts of up to 1500 tokens, 28
-// heads: 158 us (162 with last tiles of 128 slots always); 16 sequences of up to 8 new tokens and 4096 slots, 32 heads:
-// 37 us, 3.4 TB/s.
+// over 16384 slots, 64 heads of 128: 1.87 to 1.93 ms in calls one after the
+// other, 1.00 to 1.03 PFLOP/s, as the clock goes under the power limit; 12
+// prompts of up to 1500 tokens, 28 heads: 161 us; 16 sequences of up to 8 new
+// tokens and 4096 slots, 32 heads: 37 us, 3.4 TB/s.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -78,9 +78,11 @@ constexpr uint32_t kSlab = 128 * 128;  // 128 rows of 64 dims (Q, K)
 constexpr uint32_t kPageSlab = kBS * 128;  // a page's 64 dims (V)
 constexpr uint32_t kTmemCols = 512;    // S_h at h * 128, O_h at 256 + h * D
 constexpr uint32_t kColO = 256;
-// no CTA is given fewer steps than this (16 batches of few or short chunks:
-// 29.1 us in the geometric mean, 30.2 with 2, 32.5 with 4; nothing changes
-// where there is work for all CTAs)
+// no CTA is given fewer steps than this.  Few or short chunks (the first 16
+// attention batches of at most 512 rows that perf/operators.py's
+// draw(random.Random(s)) gives for s = 0, 1, ..) take 15.4 us in the geometric
+// mean, 17.1 with 2 and 19.2 with 4; nothing changes where there is work for
+// all CTAs.
 constexpr int kMinSteps = 1;
 // what an item of two tiles, or one, costs beside its tiles of slots, in the
 // eighths of a slot that AttnPolicy counts in
@@ -796,9 +798,9 @@ chunk_attention_kernel(const __grid_constant__ CUtensorMap tmQ,
 // in the order of their slots.  A block takes kJoinRows of the item's rows.
 // The pieces, their m and l, and their O are each loaded together, so that
 // the join waits for memory three times and not once per piece.  (A block
-// costs its launch even where there is nothing to join: 148 x 8 of 512 threads
-// take 0.8 us less than 148 x 16 of 256, 148 x 4 as much again, but with those
-// 96 rows over 16096 slots take 42 us and not 37.)
+// costs its launch even where there is nothing to join: the 16 batches above
+// kMinSteps take 15.4 us with 32 rows and 512 threads a block, 15.9 with 16 and
+// 256.)
 constexpr int kJoinThreads = 512;
 constexpr int kJoinRows = 32;
 

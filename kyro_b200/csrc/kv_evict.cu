@@ -100,8 +100,9 @@ __device__ int cut_before(const EvictArgs& a, const int64_t* __restrict__ contex
 // and 10.5 us with digits of 11, 11 and 10 bits, one count per value, one
 // score at a time and one CTA of 1024 threads per SM): instructions, where the
 // scores' bytes alone would take 2 us.  Three CTAs per SM where the rows are
-// short: 14 drawn batches take 18.7 us in the geometric mean, 19.7 with two and
-// 18.9 with four.
+// short: evictions (the first 14 that perf/operators.py's draw(random.Random(s))
+// gives for s = 0, 1, ..; with the copy that puts their state back) take 16.6
+// us in the geometric mean, 16.8 with two and 17.2 with four.
 __global__ void __launch_bounds__(kSelThreads, 3)
 kv_evict_select_kernel(const __grid_constant__ EvictArgs a, const __grid_constant__ LayerPtrs lp,
                        int layer0, int cached, const int64_t* __restrict__ context_lens,
@@ -461,7 +462,9 @@ kv_evict_move_kernel(const __grid_constant__ EvictArgs a, const __grid_constant_
 // numbered in batch and table order by a scan over tiles of one sequence per
 // thread, and released by all CTAs' threads in turn.  If a sequence holds a
 // shared (or invalid) block, one thread releases them all in order, so that
-// holders of one block see each other's decrements.
+// holders of one block see each other's decrements: about 0.4 us a block.  24
+// sequences x 2 layers of up to 4096 slots whose first 256 are shared by all
+// take 1615 us that way, and 85 where nothing is.
 //
 // The move lets this kernel start once the selection is complete (each of its
 // CTAs waits for that first), and reads nothing that is written here but the
@@ -690,7 +693,10 @@ int kyro_kv_evict(kyro_ctx* ctx, const kyro_evict_params* p, float* const* score
   const int64_t blocks = (int64_t)chunks * p->batch * p->num_kv_heads;
   KY_REQUIRE(blocks < (1ll << 31) && p->num_kv_heads <= 65535, "%s: batch too large", fn);
   // a row's scores are read five times: from shared memory when the longest
-  // row that the table allows fits
+  // row that the table allows fits.  (What the table allows goes by its width:
+  // 24 sequences x 2 layers of up to 4096 slots take 85 us with a table just
+  // wide enough, 91 with one of 32768 slots, whose rows leave room for one CTA
+  // per SM, and 85 with one of 131072, whose rows are read from memory.)
   const int64_t longest =
       std::min<int64_t>(p->score_slots, (int64_t)p->max_blocks_per_seq * p->block_size);
   const int cached = longest <= kRowCache ? ((int)longest + 3) / 4 * 4 : 0;

@@ -12,15 +12,17 @@
 // atomic.  An item is 256 slots of one KV head, as two tiles of 128 that
 // stay in shared memory, against the rows of as many whole tokens as 128 rows
 // hold (head in group fastest), from the first token that sees them.  One CTA
-// per SM walks its share of the items (chunk.cuh); an item that crosses a border leaves its sums to kv_scores_join_kernel, which
-// adds them in the order of the rows.  Warps:
+// per SM walks its share of the items (chunk.cuh); an item that crosses a
+// border leaves its sums to kv_scores_join_kernel, which adds them in the order
+// of the rows.  Warps:
 //   0-7, 8-15  the sums of tile 0 and of tile 1: one slot per thread and two
 //              threads per slot, which take half of a step's rows each and
 //              join their sums through the TMEM (with one, two warps on a
 //              scheduler left half of its issue slots empty: 335-350 us for
-//              2401 rows of 64 heads over 20625 slots, now 319).  All exponentials are the
-//              special-function unit's: a share of them as polynomials on the
-//              FMA pipes cost more issue slots than it saved (322-339 us)
+//              2401 rows of 64 heads over 20625 slots, now 320).  All
+//              exponentials are the special-function unit's: a share of them
+//              as polynomials on the FMA pipes cost more issue slots than it
+//              saved (322-339 us)
 //   16, 19     warp 16 walks the CTA's pieces, for all; K by TMA, a page and
 //              64 dims at a time (128-byte swizzle), the item's first and
 //              second tile.  A copy takes a warp about 75 cycles to issue, so
@@ -33,7 +35,7 @@
 // and 2048 of exponentials at D = 128, and take 2540; without the exponentials
 // they took 2250, so the loop's waits for TMEM and barriers count as much (two
 // loads in flight, by 32 columns or by 16, were slower: 340 and 332 us).  32
-// decode tokens over 130673 slots of 8 heads: 55 us, 5.0 TB/s of K.
+// decode tokens over 130673 slots of 8 heads: 57 us, 4.7 TB/s of K.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -65,8 +67,10 @@ constexpr int kKWarp = 16, kMmaWarp = 17, kQWarp = 18, kKWarp2 = 19;
 constexpr int kMaxCtas = kyro::chunk::kMaxCtas;
 constexpr uint32_t kSlab = 128 * 128;  // 128 rows of 64 dims
 constexpr uint32_t kTmemCols = 512;    // score buffer s of tile h at (2 * h + s) * 128
-// no CTA is given fewer steps than this (16 batches of few or short chunks:
-// 17.6 us in the geometric mean, 18.1 with 1, 19.0 with 4)
+// no CTA is given fewer steps than this.  Few or short chunks (the first 16
+// batches of scores of at most 512 rows that perf/operators.py's
+// draw(random.Random(s)) gives for s = 0, 1, ..) take 12.2 us in the geometric
+// mean, 12.3 with 1 and 13.4 with 4.
 constexpr int kMinSteps = 2;
 
 template <int D>

@@ -760,7 +760,8 @@ def kv_scores_add(ctx: Context, q: torch.Tensor, k_cache: torch.Tensor, lse: tor
     """kyro_kv_scores_add: the attention weight each cached slot received from
     the chunks' rows q bf16 [T, Hq, D] (lse fp32 [T, Hq] from chunk_attention
     on the same rows), added to scores fp32 [B, Hkv, slots].  In place unless
-    out is given.  Returns the scores."""
+    out is given.  Returns the scores.  A call captured into a graph should be
+    given its own workspace (kyro_kv_scores_add_workspace_size bytes)."""
     if type(ctx) is Context and ctx._calls is not None:
         ctx.bind_stream()
         r = ctx._calls.kv_scores_add(
@@ -808,7 +809,9 @@ def kv_evict(ctx: Context, budget: int, num_sink: int, num_recent: int,
     the highest scores (fp32 [B, Hkv, slots] per layer) between them, closed
     up into fresh blocks.  Returns evicted int32 [B] (slots dropped; 0 within
     the budget; -1 over it but left as it was) and fills kept int32 [layers,
-    B, Hkv, budget] with the old slots when given."""
+    B, Hkv, budget] with the old slots when given.  A call captured into a
+    graph should be given its own workspace (kyro_kv_evict_workspace_size
+    bytes)."""
     if type(ctx) is Context and ctx._calls is not None:
         ctx.bind_stream()
         r = ctx._calls.kv_evict(
