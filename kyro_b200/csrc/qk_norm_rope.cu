@@ -134,7 +134,7 @@ qk_norm_rope_kernel(const __grid_constant__ NormRopeArgs a, const uint16_t* __re
       const kyro::chunk::Seq s =
           kyro::chunk::seq_of(b, starts, context_lens, a.T, a.max_blocks * a.bs);
       const int j = t - s.start;
-      if (j >= 0 && j < s.n) {
+      if (s.n > 0 && j >= 0 && j < s.n) {
         ok = 1;
         const int slot = s.ctx + j;
         pos = positions ? positions[t] : slot;
@@ -189,7 +189,8 @@ qk_norm_rope_kernel(const __grid_constant__ NormRopeArgs a, const uint16_t* __re
         if (b0 + lane < a.B) {
           const kyro::chunk::Seq s =
               kyro::chunk::seq_of(b0 + lane, starts, context_lens, a.T, a.max_blocks * a.bs);
-          holds = t >= s.start && t - s.start < s.n;
+          // (a start may be any number where there are no rows)
+          holds = s.n > 0 && t >= s.start && t - s.start < s.n;
         }
         const uint32_t m = __ballot_sync(0xffffffffu, holds);
         if (m) last = b0 + 31 - __clz(m);

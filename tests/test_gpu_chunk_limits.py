@@ -206,3 +206,25 @@ def test_evict_short_rows_of_a_wide_table(ctx, width, sequences):
                            width_extra=width // 16)
     ev, flags = E._run(ctx, st, s, k, v, 211, 3, 50, 3, 16)
     assert flags == 0 and all((e > 0) == (n > 211) for e, n in zip(ev, lens))
+
+
+@pytest.mark.parametrize("odd", [-(1 << 31), -(1 << 31) + 5, (1 << 31) - 1])
+def test_norm_rope_write_beside_starts_of_any_size(ctx, odd):
+    """A start at the ends of its type, behind the sequence that holds the rows."""
+    from kyro_b200._lib import DEV_BAD_LENGTH
+    from kyro_b200.verify import qk_norm_rope_kv_write
+    x = R.Batch(ctx.device, [8, 8, 8], [20, 20, 20], 2, 1, 64, seed=1)
+    args = (x.block_table, x.context_lens, x.k_cache, x.v_cache, 16)
+    q, k, v = x.q[:12], x.k_new[:12], x.v_new[:12]
+
+    def call(starts):
+        out = torch.full_like(q, 7.0)
+        qk_norm_rope_kv_write(ctx, q, k, v, torch.tensor(starts, dtype=torch.int32,
+                                                         device=ctx.device), *args, q_out=out)
+        return out, ctx.device_status()
+
+    want, flags = call([0, 8, 8, 8])
+    assert flags == 0 and not (want[:8] == 7.0).all(-1).any()
+    got, flags = call([0, 8, odd, 12])
+    assert flags == DEV_BAD_LENGTH
+    assert _same(got[:8], want[:8]) and (got[8:] == 7.0).all()
